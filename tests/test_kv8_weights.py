@@ -1,0 +1,65 @@
+"""Weights and queries of very different size in the 8-bit cache's decode
+attention (``wnw_kv8_attn``), against 64 bits over the rows read back.
+
+Tolerances, derived: an output is rounded once (eps / 2 of itself, half the
+smallest subnormal number in fp16).  A weight of a full block is held in fp16,
+2^14 above the largest: off by at most 2^-11 of itself (fp16's numbers in [1, 2)
+are 2^-10 apart), and by 2^-39 of the largest below fp16's normal numbers.  A score is off by 2^-20 of the sum of its terms'
+magnitudes (fp32 sums of up to 128 exact products, three factors), which the
+weights carry twice (weight and sum) and the log-sum-exp once.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import kv8 as O
+from wnw_b200.kv8 import KV8Attention, KV8Store
+
+pytestmark = pytest.mark.gpu
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def _filled(k, v, code, page_rows=64):
+    """A store with k, v [segments, n, D] in it, and its lengths."""
+    S, n, D = k.shape
+    pages = -(-n // page_rows)
+    s = KV8Store(S, D, S * pages, pages, page_rows, code, k.dtype)
+    s.reserve(n)
+    s.append(k[:, None].cuda(), v[:, None].cuda(), torch.zeros(S, dtype=torch.int32, device="cuda"))
+    return s, torch.full((S,), n, dtype=torch.int32, device="cuda")
+
+
+def _check(store, q, n, scale, out, lse, segs):
+    eps = torch.finfo(store.dtype).eps
+    tiny = 2.0 ** -25 if store.dtype is F16 else 0.0
+    for s in segs:
+        k, v = (x.cpu().double() for x in store.dequantize(s, n))
+        x = q[s].double()
+        want, wl, pv = O.attention(x, k, v, scale)
+        ds = 2.0 ** -20 * float((x.abs() @ k.abs().t()).max()) * abs(scale)
+        tol = (eps / 2 * want.abs() * (1 + 2.0 ** -7) + (2.0 ** -11 + 2 * ds + 2.0 ** -20) * pv
+               + n * 2.0 ** -39 * float(v.abs().max()) + tiny)
+        off = (out[s].cpu().double() - want).abs()
+        assert bool((off <= tol).all()), (s, float((off / tol).max()))
+        assert bool(((lse[s].cpu().double() - wl).abs() <= ds + 2.0 ** -20 * (wl.abs() + 1)).all())
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("S,n", [(1200, 256), (1, 20), (3, 276)])
+@pytest.mark.parametrize("gap", [15.0, 17.5, 22.0, 25.0])
+def test_many_small_weights_beside_a_large_one(code, dtype, S, n, gap):
+    """One token of value zero, ``gap`` nats above all others: what comes out
+    is the others' share, whether blocks or an unfinished one hold them, over
+    several blocks a warp and over one."""
+    D = 64
+    k, v = torch.zeros(S, n, D, dtype=dtype), torch.full((S, n, D), 4096.0, dtype=dtype)
+    k[:, 0, 0] = 1.0
+    v[:, 0] = 0.0
+    store, lens = _filled(k, v, code)
+    q = torch.zeros(S, 2, D, dtype=dtype)
+    q[..., 0] = 8.0
+    out, lse = KV8Attention(store, 2, gap / 8)(q.cuda(), lens, return_lse=True)
+    _check(store, q, n, gap / 8, out, lse, range(0, S, max(1, S // 6)))
+    store.check()

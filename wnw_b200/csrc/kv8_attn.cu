@@ -21,8 +21,12 @@
 // Products: q is brought to [1, 2) per head by a power of two and held in
 // fp16 (11 bits, bf16's 8 fit), codes become fp16 exactly, so the first
 // product only rounds in its fp32 accumulation; the second takes the
-// probabilities in fp16 (2^-12 relative, 16 times below bf16's rounding of
-// the output).  Both run as m16n8k16 tensor-core products with the head
+// probabilities in fp16: 2^-11 of each, an eighth of a bf16 output's rounding
+// and as much as an fp16 one's, but random over a row's tokens.  They are held
+// 2^14 above the running maximum's, so that this is so down to 2^-28 of it and
+// what is lost below stays under 2^-39 (unscaled, 255 equal tokens 17 nats
+// under a first one of value zero vanished, at 15 nats they lost 2.5 %); the
+// values' scale takes the 2^14 back.  Both run as m16n8k16 tensor-core products with the head
 // group as n: a query token has G rows only, the tensor pipe is busy 16-19 %
 // of the time and its shape does not bound.  The value scale is applied to
 // each block's product in fp32, whatever its range.
@@ -36,6 +40,7 @@
 // time ahead of the records hides behind the append (12.5 and 45.2 us).  The
 // 16-bit kernel takes 16.8, 155.6 and 82.8 us for these lengths.
 #include <atomic>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "mma.cuh"
@@ -46,6 +51,7 @@ constexpr int kK8Threads = 256;
 constexpr int kK8Warps = 8;
 constexpr float kK8Log2e = 1.4426950408889634f;
 constexpr float kK8Ln2 = 0.6931471805599453f;
+constexpr float kK8Up = 14.f, kK8Down = 1.f / 16384.f;  // fp16 probabilities are held 2^14 up
 
 template <int D>
 constexpr int k8_stages() {
@@ -394,8 +400,8 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
       // 16-token steps in which a lane's 8 value bytes lie in order
       const int tok = 8 * (gid >> 1) + (gid & 1);
 
-      // scores -> probabilities (fp32, in sc), the running state, al0 / al1
-      auto softmax = [&](float (&sc)[2][4], float& al0, float& al1) {
+      // scores -> probabilities times 2^up (fp32, in sc), the running state, al0 / al1
+      auto softmax = [&](float (&sc)[2][4], float& al0, float& al1, float up, float down) {
         float mx0 = fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2]));
         float mx1 = fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3]));
 #pragma unroll
@@ -408,17 +414,18 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
         const float b0 = mx0 == -INFINITY ? 0.f : mx0, b1 = mx1 == -INFINITY ? 0.f : mx1;
         al0 = ex2(m0 - b0);
         al1 = ex2(m1 - b1);
+        const float u0 = b0 - up, u1 = b1 - up;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          sc[i][0] = ex2(sc[i][0] - b0);
-          sc[i][1] = ex2(sc[i][1] - b1);
-          sc[i][2] = ex2(sc[i][2] - b0);
-          sc[i][3] = ex2(sc[i][3] - b1);
+          sc[i][0] = ex2(sc[i][0] - u0);
+          sc[i][1] = ex2(sc[i][1] - u1);
+          sc[i][2] = ex2(sc[i][2] - u0);
+          sc[i][3] = ex2(sc[i][3] - u1);
         }
         m0 = mx0;
         m1 = mx1;
-        l0 = l0 * al0 + ((sc[0][0] + sc[0][2]) + (sc[1][0] + sc[1][2]));
-        l1 = l1 * al1 + ((sc[0][1] + sc[0][3]) + (sc[1][1] + sc[1][3]));
+        l0 = fmaf(l0, al0, ((sc[0][0] + sc[0][2]) + (sc[1][0] + sc[1][2])) * down);
+        l1 = fmaf(l1, al1, ((sc[0][1] + sc[0][3]) + (sc[1][1] + sc[1][3])) * down);
       };
 
       __syncwarp();
@@ -458,9 +465,11 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
           sc[i][2] = vb ? sc[i][2] * f0 : -INFINITY;
           sc[i][3] = vb ? sc[i][3] * f0 : -INFINITY;
         }
+        // probabilities as two terms of the type (8 + 8 bits for bf16, whose
+        // range needs no 2^14; 11 + 11 for fp16)
+        constexpr bool kHalf = std::is_same<T, __half>::value;
         float al0, al1;
-        softmax(sc, al0, al1);
-        // probabilities as two terms of the type (8 + 8 bits for bf16)
+        softmax(sc, al0, al1, kHalf ? kK8Up : 0.f, kHalf ? kK8Down : 1.f);
         uint32_t pb[4], pr[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -487,6 +496,7 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
           mma16816<T>(o[u], va.z, vc.z, va.w, vc.w, pb[2], pb[3]);
           mma16816<T>(o[u], va.x, vc.x, va.y, vc.y, pr[0], pr[1]);
           mma16816<T>(o[u], va.z, vc.z, va.w, vc.w, pr[2], pr[3]);
+          if constexpr (kHalf) o[u][0] *= kK8Down, o[u][1] *= kK8Down, o[u][2] *= kK8Down, o[u][3] *= kK8Down;
         }
       }
       const int xb = min(xe, cf + nfull);
@@ -524,7 +534,9 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
             sc[i][3] = c[3] * k1;
           }
           float al0, al1;
-          softmax(sc, al0, al1);
+          softmax(sc, al0, al1, kK8Up, kK8Down);
+          // (a block of values below 2^-103 loses bits of its scale here)
+          const float vs = scl.y * kK8Down;
           uint32_t pb[4];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -543,10 +555,10 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
             codes_to_half<CODE>(va.y, a0, a2);
             codes_to_half<CODE>(vc.y, a1, a3);
             mma16816<__half>(c, a0, a1, a2, a3, pb[2], pb[3]);
-            o[u][0] = fmaf(scl.y, c[0], o[u][0] * al0);
-            o[u][1] = fmaf(scl.y, c[1], o[u][1] * al1);
-            o[u][2] = fmaf(scl.y, c[2], o[u][2] * al0);
-            o[u][3] = fmaf(scl.y, c[3], o[u][3] * al1);
+            o[u][0] = fmaf(vs, c[0], o[u][0] * al0);
+            o[u][1] = fmaf(vs, c[1], o[u][1] * al1);
+            o[u][2] = fmaf(vs, c[2], o[u][2] * al0);
+            o[u][3] = fmaf(vs, c[3], o[u][3] * al1);
           }
         }
         __syncwarp();  // the stage is read
