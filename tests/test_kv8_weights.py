@@ -80,3 +80,22 @@ def test_outputs_are_rounded_once(code, dtype, D, G, n):
     out, lse = KV8Attention(store, G, D ** -0.5)(q.cuda(), lens, return_lse=True)
     _check(store, q, n, D ** -0.5, out, lse, range(4))
     store.check()
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("D,n", [(64, 96), (128, 300), (128, 32)])
+def test_small_dimensions_beside_a_large_one(code, dtype, D, n):
+    """Queries whose largest dimension meets only zeros: the others, 2^-20 of
+    it, are all that the scores are made of."""
+    g = torch.Generator().manual_seed(n)
+    k, v = (torch.randn(3, n, D, generator=g).to(dtype) for _ in range(2))
+    k[..., 0] = 0.0
+    bits = 128 if dtype is BF16 else 1024
+    q = (1 + torch.randint(0, bits, (3, 4, D), generator=g) / bits) * 2.0 ** -10
+    q = (q * (1 - 2 * torch.randint(0, 2, q.shape, generator=g))).to(dtype)
+    q[..., 0] = 1024.0
+    store, lens = _filled(k, v, code)
+    out, lse = KV8Attention(store, 4, 2.0 ** 8)(q.cuda(), lens, return_lse=True)
+    _check(store, q, n, 2.0 ** 8, out, lse, range(3))
+    store.check()

@@ -18,9 +18,11 @@
 // and parts of several CTAs through `partials`, slice by slice, by the last
 // warp to arrive, in the line's order: results repeat bit for bit.
 //
-// Products: q is brought to [1, 2) per head by a power of two and held in
-// fp16 (11 bits, bf16's 8 fit), codes become fp16 exactly, so the first
-// product only rounds in its fp32 accumulation; the second takes the
+// Products: q is brought to [2^15, 2^16) per head by a power of two and held
+// in fp16: exact for fp16 models, for bf16 ones down to 2^-32 of the head's
+// largest dimension (11 bits, bf16's 8 fit; what fp16 cannot hold below that
+// is under 2^-40 of it).  Codes become fp16 exactly, so the first product
+// rounds in its fp32 accumulation only.  The second takes the
 // probabilities as two fp16 terms, 22 bits, so outputs are as near as with
 // fp32 ones (one term, 2^-11 of each: as much as an fp16 output's own
 // rounding, an eighth of a bf16 one's; 1 to 3 % faster: two requests of 120k
@@ -376,17 +378,17 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
         for (int e = 0; e < D / 4; ++e) mx = max(mx, __float_as_uint(qf[e]) & 0x7fffffffu);
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        int e = static_cast<int>(mx >> 23) - 127;
-        e = mx >= 0x7f800000u || mx == 0 ? 0 : min(126, max(-126, e));
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-        fac = a.scale * kK8Log2e * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        // (an infinity or a NaN comes through as it is; the factor back stays a normal number)
+        const int e = mx >= 0x7f800000u || mx == 0 ? 0 : min(120, 142 - static_cast<int>(mx >> 23));
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        fac = a.scale * kK8Log2e * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
 #pragma unroll
         for (int j = 0; j < D / 64; ++j)
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const float* f = qf + 16 * j + 4 * u;
-            qb[4 * j + u][0] = pack2<__half>(f[0] * down, f[1] * down);
-            qb[4 * j + u][1] = pack2<__half>(f[2] * down, f[3] * down);
+            qb[4 * j + u][0] = pack2<__half>(f[0] * up, f[1] * up);
+            qb[4 * j + u][1] = pack2<__half>(f[2] * up, f[3] * up);
           }
       }
       // the two heads of a lane's accumulators
