@@ -719,6 +719,7 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
     }
   }
   const uint32_t lasts = __ballot_sync(0xffffffffu, last);
+  __syncwarp();  // what lanes 0 and 1 acquired orders the other lanes' loads of partials too (a vote orders no memory)
 #pragma unroll 1
   for (int e = 0; e < 2; ++e) {
     if (!(lasts >> e & 1u)) continue;
