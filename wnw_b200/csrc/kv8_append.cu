@@ -212,9 +212,10 @@ __global__ void __launch_bounds__(kApThreads, RESIDENT) kv8_append_kernel(const 
         const int j0 = L / kKv8Block, j = j0 + block, jl = end / kKv8Block;
         const bool clash = role != kApQueries && (L % kKv8Block) != 0 && (end % kKv8Block) != 0 && jl - j0 >= 2 &&
                            ((jl - j0) & 1) == 0;
-        if (j * kKv8Block < end && !(clash && j == jl)) jb[0] = j;
+        // (numbers of blocks: a block behind the last one may begin beyond 31 bits)
+        if (j <= (end - 1) / kKv8Block && !(clash && j == jl)) jb[0] = j;
         if (clash && j == j0) jb[1] = jl;
-        if (jb[0] >= 0 && (j + 1) * kKv8Block <= end && role != kApQueries) {
+        if (jb[0] >= 0 && j < jl && role != kApQueries) {
           const int page = __ldg(st.page_table + int64_t(seg) * st.max_pages + (j >> p.page_shift));
           if (page < 0 || page >= st.num_pages) {
             atomicOr(st.err, WNW_DEVERR_BAD_INDEX);
