@@ -3,11 +3,18 @@ documentation allows: numbers near 31 bits, outputs that share memory,
 derivatives, growth."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+from oracle import kv8 as O
 from wnw_b200.kv8 import KV8Store
+from wnw_b200.rotary import Rotary
 
 gpu = pytest.mark.gpu
 BF16 = torch.bfloat16
+
+
+def _freq(half, base=1e4):
+    return (base ** (-torch.arange(half, dtype=torch.float64) / half)).float()
 
 
 @gpu
@@ -34,3 +41,56 @@ def test_append_behind_two_billion_rows(left):
         want[0, at, rows % 32] = 1
         assert torch.equal(s.tail_k, want) and torch.equal(s.tail_v, want.transpose(2, 3))
     assert bool((s.pool == 7).all())
+
+
+# ------------------------------------------------- derivatives of the rotation
+
+class _OnTheCpu(Rotary):
+    """The rotation with its launch replaced by the formula, for what autograd
+    does around it."""
+
+    def _launch(self, q, k, positions, inverse, out, stream):
+        axis = self.axis.tolist()
+        return tuple(None if x is None else O.rotate(x, positions, self.inv_freq, axis, inverse).to(x.dtype)
+                     for x in (q, k))
+
+
+def _forward_derivatives(rotary, device):
+    g = torch.Generator().manual_seed(2)
+    q, tq, gq = (torch.randn(2, 3, 5, 64, generator=g).to(device) for _ in range(3))
+    k, tk, gk = (torch.randn(2, 2, 5, 64, generator=g).to(device) for _ in range(3))
+    pos = torch.randint(0, 900, (2, 2, 5), generator=g).to(device)
+    want = rotary(tq, tk, pos)
+    for inverse in (False, True):
+        turned = rotary(tq, tk, pos, inverse=inverse)
+        with forward_ad.dual_level():
+            for grads in (False, True):
+                a, b = (x.clone().requires_grad_(grads) for x in (q, k))
+                yq, yk = rotary(forward_ad.make_dual(a, tq), forward_ad.make_dual(b, tk), pos, inverse=inverse)
+                assert torch.equal(forward_ad.unpack_dual(yq).tangent, turned[0])
+                assert torch.equal(forward_ad.unpack_dual(yk).tangent, turned[1])
+                if grads:
+                    da, db = torch.autograd.grad([forward_ad.unpack_dual(y).primal for y in (yq, yk)], (a, b), (gq, gk))
+                    back = rotary(gq, gk, pos, inverse=not inverse)
+                    assert torch.equal(da, back[0]) and torch.equal(db, back[1])
+    with forward_ad.dual_level():
+        # one of the two, a broadcast tangent, no gradients recorded
+        with torch.no_grad():
+            yq, yk = rotary(q, forward_ad.make_dual(k, tk), pos)
+        assert not forward_ad.unpack_dual(yq).tangent.any() and torch.equal(forward_ad.unpack_dual(yk).tangent, want[1])
+        ones = torch.ones(1, device=device).expand(q.shape)
+        y, none = rotary(forward_ad.make_dual(q, ones), None, pos)
+        assert none is None and torch.equal(forward_ad.unpack_dual(y).tangent, rotary(ones.contiguous(), None, pos)[0])
+        with pytest.raises(ValueError, match="gradients"):
+            rotary(forward_ad.make_dual(q, tq), None, pos, out=(torch.empty_like(q), None))
+        y, _ = rotary(q, None, pos)
+        assert forward_ad.unpack_dual(y).tangent is None
+
+
+def test_rotary_forward_derivatives_are_carried():
+    _forward_derivatives(_OnTheCpu(_freq(32), sections=(10, 22)), "cpu")
+
+
+@gpu
+def test_rotary_forward_derivatives():
+    _forward_derivatives(Rotary(_freq(32).cuda(), sections=(10, 22)), "cuda")

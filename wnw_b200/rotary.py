@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from wnw_b200 import native as N
 from wnw_b200.kernels import LAUNCHES, check_device_error
@@ -84,8 +85,9 @@ class Rotary:
         above (up to 2^51) they carry a rounding to 64 bits.  ``inverse``
         applies the transposed rotation: the gradient of the forward one.  ``out``: (q, k) to write, which may
         be the inputs themselves.  ``stream``: launch there, behind what the
-        caller made it wait for.  Differentiable with respect to q and k."""
-        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+        caller made it wait for.  Differentiable with respect to q and k,
+        backward and forward (dual tensors)."""
+        if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k):
             if out is not None or stream is not None:
                 raise ValueError("out and stream cannot be given where gradients are wanted")
             return _Rotate.apply(self, q, k, positions, inverse)
@@ -152,29 +154,47 @@ class Rotary:
 
 
 class _Rotate(torch.autograd.Function):
-    """The rotation is linear, its gradient the transposed rotation."""
+    """The rotation is linear: its gradient is the transposed rotation, its
+    forward derivative the rotation of the tangents."""
 
     @staticmethod
     def forward(ctx, rotary, q, k, positions, inverse):
         ctx.rotary, ctx.inverse = rotary, inverse
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
-        return rotary._launch(q, k, positions, inverse, None, None)
+        ctx.positions = positions
+        out = rotary._launch(q, k, positions, inverse, None, None)
+        ctx.like = [None if y is None else (y.shape, y.dtype, y.device) for y in out]
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gq, gk):
         pos, = ctx.saved_tensors
-        r = ctx.rotary
-        q = k = None
         gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad[1:3]))
-        if gq is not None and gk is not None:
-            q, k = r._launch(_rows(gq), _rows(gk), pos, not ctx.inverse, None, None)
-        elif gq is not None:
-            q, _ = r._launch(_rows(gq), None, pos, not ctx.inverse, None, None)
-        elif gk is not None:
-            k, _ = r._launch(_rows(gk), None, pos, not ctx.inverse, None, None)
-        return None, q, k, None, None
+        return None, *_some(ctx.rotary, gq, gk, pos, not ctx.inverse), None, None
+
+    @staticmethod
+    def jvp(ctx, _rotary, tq, tk, _positions, _inverse):
+        turned = _some(ctx.rotary, tq, tk, ctx.positions, ctx.inverse)
+        # (an output whose input has no tangent is given a zero one: autograd takes no None for it)
+        return tuple(t if t is not None or y is None else torch.zeros(y[0], dtype=y[1], device=y[2])
+                     for t, y in zip(turned, ctx.like))
+
+
+def _dual(*tensors):
+    """Whether one of them carries a forward derivative."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _some(rotary, q, k, positions, inverse):
+    """The rotation of derivatives, either of which may be None."""
+    if q is not None:
+        return rotary._launch(_rows(q), None if k is None else _rows(k), positions, inverse, None, None)
+    if k is not None:
+        return None, rotary._launch(_rows(k), None, positions, inverse, None, None)[0]
+    return None, None
 
 
 def _rows(x):
