@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 from oracle import kv8 as O
-from wnw_b200.kv8 import KV8Store
+from wnw_b200.kv8 import KV8Attention, KV8Store
 from wnw_b200.rotary import Rotary
 
 gpu = pytest.mark.gpu
@@ -94,3 +94,44 @@ def test_rotary_forward_derivatives_are_carried():
 @gpu
 def test_rotary_forward_derivatives():
     _forward_derivatives(Rotary(_freq(32).cuda(), sections=(10, 22)), "cuda")
+
+
+# -------------------------------------------------------- what calls write into
+
+def _stale(saved, write):
+    """A backward pass that needs ``saved`` as it was, after ``write``."""
+    w = torch.ones(saved.shape, device=saved.device, dtype=torch.float32, requires_grad=True)
+    y = (w * saved).sum() if saved.dtype is torch.float32 else (w.to(saved.dtype) * saved).sum()
+    with torch.no_grad():
+        write()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@gpu
+def test_backward_passes_refuse_what_calls_have_overwritten():
+    r = Rotary(_freq(32).cuda())
+    pos = torch.arange(3, device="cuda")[None]
+    q, k = torch.randn(1, 4, 3, 64, device="cuda"), torch.randn(1, 2, 3, 64, device="cuda")
+    _stale(q, lambda: r(q, None, pos, out=(q, None)))
+    _stale(k, lambda: r(q, k, pos, out=(torch.empty_like(q), k)))
+    s = KV8Store(2, 64, 4, 2, page_rows=32)
+    s.reserve(64)
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    qb, kb = q.to(BF16), k.to(BF16)
+    _stale(qb, lambda: s.append(kb, kb, lens, rotary=r, positions=pos, q=qb, q_out=qb))
+    for held in (s.tail_k, s.tail_v, s.scales()):
+        _stale(held, lambda: s.append(kb, kb, lens))
+    att, out = KV8Attention(s, 2, 0.1), torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
+    _stale(out, lambda: att(qb[0, :, 0].reshape(2, 2, 64).contiguous(), lens, out=out))
+    # what a call only reads stays good, and results made in the call are new
+    w = torch.ones_like(q, requires_grad=True)
+    y = (w * q).sum()
+    with torch.no_grad():
+        r(q, k, pos)
+    y.backward()
+    assert torch.equal(w.grad, q)
+    with torch.inference_mode():
+        x = q.clone()
+        r(x, None, pos, out=(x, None))
+    assert torch.equal(x, r(q, None, pos)[0])

@@ -23,7 +23,7 @@ import torch
 
 from wnw_b200 import native as N
 from wnw_b200.kernels import check_device_error
-from wnw_b200.rotary import dense, distinct, keep_for, launch, made_on, rows
+from wnw_b200.rotary import dense, distinct, keep_for, launch, made_on, rows, written
 
 BLOCK = N.KV8_BLOCK
 _CONTIGUOUS = torch.contiguous_format
@@ -204,6 +204,7 @@ class KV8Store:
             q_in, q_to = q.data_ptr(), q_out.data_ptr()
         launch(index, stream, _APPEND, "wnw_kv8_append_step", base[1], k.data_ptr(), v.data_ptr(), lengths, first, many,
                pos, q_in, q_to)
+        written(self.pool, self.tail_k, self.tail_v, q_out)
         if stream is not None:
             keep_for(stream, k, v, seg_len, starts, counts, positions, q, q_out, *self._tensors())
             if rotary is not None:
@@ -352,6 +353,7 @@ class KV8Attention:
             fresh = -1
         elif not 0 <= fresh < 1 << 31:
             raise ValueError(f"fresh {fresh}: a number of tokens")
+        given = out
         if out is None:
             out = made_on(stream, s._index, torch.empty_like, q)
         elif out.shape != shape or out.dtype is not s.dtype or not out.is_contiguous() \
@@ -360,6 +362,8 @@ class KV8Attention:
         lse = made_on(stream, s._index, torch.empty_like, self._lse_like) if return_lse else None
         launch(s._index, stream, _ATTEND, "wnw_kv8_attn_step", self._args, q.data_ptr(), lengths, out.data_ptr(),
                lse.data_ptr() if return_lse else None, fresh)
+        if given is not None:
+            written(given)
         if stream is not None:
             keep_for(stream, q, seg_len, out, lse, self.partials, self.counters, *s._tensors())
         return (out, lse) if return_lse else out

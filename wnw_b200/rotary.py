@@ -15,6 +15,7 @@ import ctypes as C
 
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from wnw_b200 import native as N
 from wnw_b200.kernels import LAUNCHES, check_device_error
@@ -115,6 +116,8 @@ class Rotary:
                 raise ValueError(f"a tensor on {t.device}: the rotation is on {self.device} and needs a CUDA device")
         launch(index, stream, _ROTARY, "wnw_rotary_step", base[1], q.data_ptr(), qo.data_ptr(),
                None if k is None else k.data_ptr(), None if ko is None else ko.data_ptr(), positions.data_ptr())
+        if out is not None:
+            written(qo, ko)
         if stream is not None:
             keep_for(stream, q, k, qo, ko, positions, self._freq64, self.axis, self.err)
         return qo, ko
@@ -262,6 +265,12 @@ def made_on(stream, index, make, *args, **kw):
     if t.is_cuda:
         t.record_stream(torch.cuda.current_stream(index))
     return t
+
+
+def written(*tensors):
+    """Tell autograd that a launch has written into the caller's tensors: what
+    was saved of them for a backward pass is refused there."""
+    increment_version([t for t in tensors if t is not None])
 
 
 def keep_for(stream, *tensors):
