@@ -135,3 +135,34 @@ def test_backward_passes_refuse_what_calls_have_overwritten():
         x = q.clone()
         r(x, None, pos, out=(x, None))
     assert torch.equal(x, r(q, None, pos)[0])
+
+
+def test_outputs_that_carry_derivatives_are_refused():
+    r, q, pos = Rotary(_freq(32)), torch.zeros(1, 4, 3, 64), torch.zeros(1, 3, dtype=torch.int64)
+    leaf = torch.zeros(1, 4, 3, 64, requires_grad=True)
+    for out in (leaf, leaf * 2):
+        with pytest.raises(ValueError, match="carries derivatives"):
+            r(q, None, pos, out=(out, None))
+        with pytest.raises(ValueError, match="carries derivatives"):
+            r(q, q, pos, out=(torch.zeros_like(q), out))
+        with torch.no_grad(), pytest.raises(ValueError, match="CUDA device"):  # as far as the device
+            r(q, None, pos, out=(out, None))
+    with forward_ad.dual_level(), pytest.raises(ValueError, match="carries derivatives"):
+        r(q, None, pos, out=(forward_ad.make_dual(torch.zeros_like(q), q), None))
+
+
+@gpu
+def test_outputs_of_the_cache_that_carry_derivatives_are_refused():
+    s = KV8Store(2, 64, 2, 1, page_rows=32)
+    s.reserve(32)
+    lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+    kv = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda")
+    q, pos = torch.zeros(1, 4, 3, 64, dtype=BF16, device="cuda"), torch.zeros(1, 3, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="carries derivatives"):
+        s.append(kv, kv, lens, rotary=Rotary(_freq(32).cuda()), positions=pos, q=q, q_out=torch.empty_like(q).requires_grad_())
+    one = torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
+    with pytest.raises(ValueError, match="carries derivatives"):
+        KV8Attention(s, 2, 0.1)(one, lens, out=torch.empty_like(one).requires_grad_())
+    with torch.no_grad():
+        KV8Attention(s, 2, 0.1)(one, lens, out=torch.empty_like(one).requires_grad_())
+    s.check()

@@ -23,7 +23,7 @@ import torch
 
 from wnw_b200 import native as N
 from wnw_b200.kernels import check_device_error
-from wnw_b200.rotary import dense, distinct, keep_for, launch, made_on, rows, written
+from wnw_b200.rotary import dense, distinct, keep_for, launch, made_on, plain, rows, written
 
 BLOCK = N.KV8_BLOCK
 _CONTIGUOUS = torch.contiguous_format
@@ -199,8 +199,10 @@ class KV8Store:
             if q_out is None:
                 make = torch.empty_like if counts is None else torch.zeros_like
                 q_out = made_on(stream, index, make, q, memory_format=_CONTIGUOUS)
-            elif q_out.get_device() != index:
-                self._check_device(q_out)
+            else:
+                plain(q_out)
+                if q_out.get_device() != index:
+                    self._check_device(q_out)
             q_in, q_to = q.data_ptr(), q_out.data_ptr()
         launch(index, stream, _APPEND, "wnw_kv8_append_step", base[1], k.data_ptr(), v.data_ptr(), lengths, first, many,
                pos, q_in, q_to)
@@ -359,6 +361,8 @@ class KV8Attention:
         elif out.shape != shape or out.dtype is not s.dtype or not out.is_contiguous() \
                 or out.get_device() != s._index:
             raise ValueError(f"out {tuple(out.shape)} {out.dtype}: expected contiguous {shape} {s.dtype}")
+        else:
+            plain(out)
         lse = made_on(stream, s._index, torch.empty_like, self._lse_like) if return_lse else None
         launch(s._index, stream, _ATTEND, "wnw_kv8_attn_step", self._args, q.data_ptr(), lengths, out.data_ptr(),
                lse.data_ptr() if return_lse else None, fresh)

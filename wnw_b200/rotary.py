@@ -92,6 +92,8 @@ class Rotary:
             if out is not None or stream is not None:
                 raise ValueError("out and stream cannot be given where gradients are wanted")
             return _Rotate.apply(self, q, k, positions, inverse)
+        if out is not None:
+            plain(*out)
         return self._launch(q, k, positions, inverse, out, stream)
 
     def _launch(self, q, k, positions, inverse, out, stream):
@@ -265,6 +267,13 @@ def made_on(stream, index, make, *args, **kw):
     if t.is_cuda:
         t.record_stream(torch.cuda.current_stream(index))
     return t
+
+
+def plain(*outputs):
+    """Refuse to write into tensors that carry derivatives: the call would not
+    be part of them."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in outputs) or _dual(*outputs):
+        raise ValueError("a given output carries derivatives: write into a detached one, or under no_grad")
 
 
 def written(*tensors):
