@@ -1,13 +1,15 @@
 """Calls of the 8-bit cache and the rotation at the borders of what their
 documentation allows: numbers near 31 bits, outputs that share memory,
 derivatives, growth."""
+import random
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from oracle import kv8 as O
 from wnw_b200.kv8 import KV8Attention, KV8Store
-from wnw_b200.rotary import Rotary
+from wnw_b200.rotary import Apart, Rotary
 
 gpu = pytest.mark.gpu
 BF16 = torch.bfloat16
@@ -165,4 +167,84 @@ def test_outputs_of_the_cache_that_carry_derivatives_are_refused():
         KV8Attention(s, 2, 0.1)(one, lens, out=torch.empty_like(one).requires_grad_())
     with torch.no_grad():
         KV8Attention(s, 2, 0.1)(one, lens, out=torch.empty_like(one).requires_grad_())
+    s.check()
+
+
+# ----------------------------------------------------- outputs that share memory
+
+def test_shared_elements_are_found():
+    """Against the sets of elements themselves, over random views of one buffer."""
+    rnd, found = random.Random(4), [0, 0]
+    buf = torch.zeros(4000)
+    for _ in range(2000):
+        B, H, n, D = (rnd.randint(1, 3) for _ in range(4))
+        pad = [rnd.randint(0, 2) for _ in range(3)]
+        order = rnd.sample(range(3), 3)
+        strides, span = [0, 0, 0], D + pad[0]
+        for d in order:
+            strides[d] = span
+            span *= (B, H, n)[d] + rnd.randint(0, 3)
+        a, b = (buf.as_strided((B, h, n, D), (*strides, 1), rnd.randint(0, 40)) for h in (H, rnd.randint(1, H)))
+        ids = [set((torch.arange(4000).as_strided(x.shape, x.stride(), x.storage_offset())).flatten().tolist())
+               for x in (a, b)]
+        share = bool(ids[0] & ids[1])
+        found[share] += 1
+        for x, y in ((a, b), (b, a)):
+            check, at = Apart(("x", x, None), ("y", None, y)), (x.data_ptr(), None, None, y.data_ptr())
+            for _ in range(2):
+                if share:
+                    with pytest.raises(ValueError, match="shares memory"):
+                        check(*at)
+                else:
+                    check(*at)
+    assert min(found) > 200
+
+
+def test_outputs_that_share_memory_with_other_tensors_are_refused():
+    r, pos = Rotary(_freq(32)), torch.zeros(2, 5, dtype=torch.int64)
+    qkv = torch.zeros(2, 5, 8, 64).transpose(1, 2)
+    q, k, v = qkv.split([4, 2, 2], 1)
+    two = torch.zeros(2, 4, 6, 64)
+    for ins, outs in (((k, v), (v, k)), ((k, v), (k, k)), ((k, v), (torch.zeros_like(k), k)), ((k, v), (v, torch.zeros_like(v))),
+                      ((two[:, :, :5], None), (two[:, :, 1:], None)),
+                      ((two[:, :, :4], None), (two.view(-1)[:2 * 4 * 4 * 64].view(2, 4, 4, 64), None))):
+        with pytest.raises(ValueError, match="shares memory"):
+            r(*ins, pos[:, :ins[0].shape[2]], out=outs)
+    one = torch.zeros(1, 4, 1, 64)
+    for ins, outs in (((q, k), (q, k)), ((q, k), (q, torch.zeros_like(k))), ((q, None), (torch.zeros_like(q), None)),
+                      ((one, None), (one.as_strided(one.shape, (7, 64, 9, 1)), None))):
+        with pytest.raises(ValueError, match="CUDA device"):  # as far as the device
+            r(*ins, pos[:ins[0].shape[0], :ins[0].shape[2]], out=outs)
+
+
+def test_query_rows_that_share_memory_with_keys_are_refused():
+    s, lens = KV8Store(4, 64, 4, 1, page_rows=64, device="cpu"), torch.zeros(4, dtype=torch.int32)
+    x = torch.zeros(2, 3, 8, 64).bfloat16().transpose(1, 2)
+    q, k, v = x.split([4, 2, 2], 1)
+    args = dict(rotary=Rotary(_freq(32)), positions=torch.zeros(1, 2, 3, dtype=torch.int64), q=q)
+    for out in (x[:, 1:5], x[:, 2:6], x[:, 4:], x[:, 3:7]):
+        with pytest.raises(ValueError, match="shares memory"):
+            s.append(k, v, lens, q_out=out, **args)
+    for out in (q, torch.zeros_like(q)):
+        with pytest.raises(ValueError, match="CUDA device"):
+            s.append(k, v, lens, q_out=out, **args)
+
+
+@gpu
+def test_outputs_in_place_and_refused_ones_on_the_gpu():
+    """In place within one packed buffer: the bits of separate outputs."""
+    r, pos = Rotary(_freq(32).cuda()), torch.arange(10, device="cuda").view(2, 5)
+    qkv = torch.randn(2, 5, 8, 64, device="cuda").to(BF16).transpose(1, 2)
+    q, k, v = qkv.split([4, 2, 2], 1)
+    want, left = r(q, k, pos), v.clone()
+    with pytest.raises(ValueError, match="shares memory"):
+        r(k, v, pos, out=(v, k))
+    r(q, k, pos, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, left)
+    s = KV8Store(4, 64, 4, 1, page_rows=32)
+    s.reserve(32)
+    att, lens, x = KV8Attention(s, 2, 0.1), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.randn(5, 2, 64, device="cuda").to(BF16)
+    with pytest.raises(ValueError, match="shares memory"):
+        att(x[:4], lens, out=x[1:])
+    assert not att(x[:4], lens, out=x[:4])[:].any()  # q itself: no rows, zeros
     s.check()

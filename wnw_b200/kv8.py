@@ -23,7 +23,7 @@ import torch
 
 from wnw_b200 import native as N
 from wnw_b200.kernels import check_device_error
-from wnw_b200.rotary import dense, distinct, keep_for, launch, made_on, plain, rows, written
+from wnw_b200.rotary import Apart, dense, distinct, keep_for, launch, made_on, plain, rows, written
 
 BLOCK = N.KV8_BLOCK
 _CONTIGUOUS = torch.contiguous_format
@@ -159,8 +159,8 @@ class KV8Store:
         are starts[b] ... starts[b] + counts[b] of the n, ``max_count`` (host)
         at least the largest count.  ``rotary`` (a ``Rotary``) with
         ``positions`` [axes, B, n] rotates the keys before they are held, and
-        ``q`` [B, q heads, n, D] into the returned tensor (``q_out`` or a new
-        one, contiguous; where a sample has no token a new one is zero and a
+        ``q`` [B, q heads, n, D] into the returned tensor (``q_out``, which
+        may be q and shares no memory with k and v, or a new one, contiguous; where a sample has no token a new one is zero and a
         given one is left as it is).  Returns None without q.  ``stream``:
         launch there, behind what the caller made it wait for.  Problems on the
         device (a segment beyond its pages, an index out of range) set bits
@@ -178,6 +178,9 @@ class KV8Store:
             if len(self._appends) >= 64:
                 self._appends.clear()
             self._appends[key] = base
+        if q_out is not None:
+            plain(q_out)
+            base[2](q_out.data_ptr(), q.data_ptr(), None, k.data_ptr(), None, v.data_ptr())
         index = self._index
         if index < 0 or k.get_device() != index or v.get_device() != index:
             self._check_device(k, v)
@@ -199,10 +202,8 @@ class KV8Store:
             if q_out is None:
                 make = torch.empty_like if counts is None else torch.zeros_like
                 q_out = made_on(stream, index, make, q, memory_format=_CONTIGUOUS)
-            else:
-                plain(q_out)
-                if q_out.get_device() != index:
-                    self._check_device(q_out)
+            elif q_out.get_device() != index:
+                self._check_device(q_out)
             q_in, q_to = q.data_ptr(), q_out.data_ptr()
         launch(index, stream, _APPEND, "wnw_kv8_append_step", base[1], k.data_ptr(), v.data_ptr(), lengths, first, many,
                pos, q_in, q_to)
@@ -214,8 +215,8 @@ class KV8Store:
         return q_out
 
     def _append_args(self, k, v, ragged, max_count, q, rotary, positions, q_out):
-        """(argument block without pointers, a reference to it) of one append
-        geometry, checked."""
+        """(argument block without pointers, a reference to it, the check of a
+        given output's address) of one append geometry, checked."""
         shape, dtype = k.shape, self.dtype
         if len(shape) != 4 or v.shape != shape or k.dtype != dtype or v.dtype != dtype:
             raise ValueError(f"k {tuple(k.shape)} {k.dtype} and v {tuple(v.shape)} {v.dtype}: expected "
@@ -251,7 +252,7 @@ class KV8Store:
             raise ValueError("q_out without q")
         a = N.Kv8AppendArgs(self._desc, B, H, n, max_count, None, None, None, *rows(k, "k", shape),
                             *rows(v, "v", shape), *queries, rope)
-        return a, C.byref(a)
+        return a, C.byref(a), None if q_out is None else Apart(("q_out", q_out, q), ("k", None, k), ("v", None, v))
 
     def _tensors(self):
         return self.pool, self.page_table, self.tail_k, self.tail_v, self.err
@@ -331,6 +332,7 @@ class KV8Attention:
         self._base = N.Kv8AttnArgs(store._desc, self.group, None, None, None, None, self.scale,
                                    self.partials.data_ptr(), self.partials.numel(), self.counters.data_ptr(), -1)
         self._args = C.byref(self._base)
+        self._bytes = store.num_segs * self.group * store.head_dim * store.tail_k.element_size()
         self._lse_like = torch.empty(self.shape[:2], dtype=torch.float32, device=store.device)
 
     def __call__(self, q, seg_len, *, out=None, return_lse=False, fresh=None, stream=None):
@@ -363,6 +365,8 @@ class KV8Attention:
             raise ValueError(f"out {tuple(out.shape)} {out.dtype}: expected contiguous {shape} {s.dtype}")
         else:
             plain(out)
+            if 0 < abs(out.data_ptr() - q.data_ptr()) < self._bytes:
+                raise ValueError("out: shares memory with other rows of q")
         lse = made_on(stream, s._index, torch.empty_like, self._lse_like) if return_lse else None
         launch(s._index, stream, _ATTEND, "wnw_kv8_attn_step", self._args, q.data_ptr(), lengths, out.data_ptr(),
                lse.data_ptr() if return_lse else None, fresh)

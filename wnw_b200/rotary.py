@@ -84,8 +84,8 @@ class Rotary:
         dimensions of any stride; positions [axes, B, n] ([B, n] with one
         axis), int32 or int64: below 2^29 in magnitude their angles are exact,
         above (up to 2^51) they carry a rounding to 64 bits.  ``inverse``
-        applies the transposed rotation: the gradient of the forward one.  ``out``: (q, k) to write, which may
-        be the inputs themselves.  ``stream``: launch there, behind what the
+        applies the transposed rotation: the gradient of the forward one.  ``out``: (q, k) to write, each of
+        which may be its own input and shares no memory with the other tensors.  ``stream``: launch there, behind what the
         caller made it wait for.  Differentiable with respect to q and k,
         backward and forward (dual tensors)."""
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k):
@@ -109,6 +109,8 @@ class Rotary:
                 self._calls.clear()
             self._calls[key] = base
         index = self._index
+        if out is not None:
+            base[2](qo.data_ptr(), q.data_ptr(), None if ko is None else ko.data_ptr(), None if k is None else k.data_ptr())
         if out is None:
             qo = made_on(stream, index, torch.empty_like, q, memory_format=torch.contiguous_format)
             if k is not None:
@@ -125,8 +127,8 @@ class Rotary:
         return qo, ko
 
     def _call_args(self, q, k, positions, inverse, out):
-        """(argument block without pointers, a reference to it) of one
-        geometry, checked."""
+        """(argument block without pointers, a reference to it, the check of
+        given outputs' addresses) of one geometry, checked."""
         if q.dim() != 4 or q.dtype not in _TYPES:
             raise ValueError(f"q {tuple(q.shape)} {q.dtype}: expected [B, heads, n, D] in fp32, fp16 or bf16")
         B, Hq, n, D = q.shape
@@ -152,7 +154,7 @@ class Rotary:
             strides += (*rows(x, "qk"[i], x.shape), *to)
         a = N.RotaryArgs(N.dtype_code(q.dtype), D, B, n, Hq, 0 if k is None else k.shape[1], *strides,
                          self.rope(positions, B, n), bool(inverse), self._err_ptr)
-        return a, C.byref(a)
+        return a, C.byref(a), None if out is None else Apart(("q_out", out[0], q), ("k_out", out[1], k))
 
     def check(self):
         check_device_error(self.err)
@@ -230,6 +232,66 @@ def distinct(t, name):
         if stride < span:
             raise ValueError(f"{name}: elements share memory (shape {tuple(t.shape)}, strides {t.stride()})")
         span = stride * n
+
+
+class Apart:
+    """Refuses the outputs of one geometry's calls that share memory with
+    another output, with another's input, or with their own at other elements.
+    From (name, output, its input) tensors; a call brings their addresses, in
+    the same order, None where there is no tensor."""
+
+    def __init__(self, *triples):
+        layouts = [(name, w, t) for name, *ts in triples for w, t in zip((True, False), ts)]
+        self._pairs = []
+        for j, (_, wj, b) in enumerate(layouts):
+            for i, (name, wi, a) in enumerate(layouts[:j]):
+                if a is None or b is None or not (wi or wj) or not (a.numel() and b.numel()):
+                    continue
+                own = i == j - 1 and j % 2 == 1 and all(
+                    s == t or n == 1 for s, t, n in zip(a.stride(), b.stride(), a.shape))
+                la, lb = ((t.shape, t.stride(), t.element_size()) for t in (a, b))
+                self._pairs.append((i, j, _span(la), _span(lb), own, {}, la, lb, name))
+
+    def __call__(self, *at):
+        for i, j, after, before, own, known, la, lb, name in self._pairs:
+            d = at[j] - at[i]
+            if -before < d < after and not (own and d == 0):
+                meet = known.get(d)
+                if meet is None:
+                    if len(known) > 64:
+                        known.clear()
+                    meet = known[d] = _meet(la, lb, d)
+                if meet:
+                    raise ValueError(f"{name}: shares memory with another tensor of the call")
+
+
+def _span(layout):
+    shape, strides, size = layout
+    return size * (1 + sum(s * (n - 1) for s, n in zip(strides, shape)))
+
+
+def _meet(a, b, distance):
+    """Whether two tensors (shape, strides, bytes an element) whose starts are
+    so many bytes apart have an element in common, given that what they span
+    does.  Exact where the strides are the same (views of one buffer), else
+    taken to be so."""
+    (na, sa, e), (nb, sb, f) = a, b
+    if e != f or distance % e or len(na) != len(nb) \
+            or any(x > 1 and y > 1 and s != t for s, t, x, y in zip(sa, sb, na, nb)):
+        return True
+    # a's element i and b's element j are one where the sum of stride x (i - j) is the distance of their starts
+    dims = sorted(((s if x > 1 else t, y - 1, x - 1) for s, t, x, y in zip(sa, sb, na, nb) if x > 1 or y > 1),
+                  reverse=True)
+
+    def reach(at, rest):
+        if at == len(dims) or dims[at][0] == 0:
+            return rest == 0
+        stride, down, up = dims[at]
+        low, high = (sum(d[0] * d[w] for d in dims[at + 1:]) for w in (1, 2))
+        first, last = -((high - rest) // stride), (rest + low) // stride
+        return any(reach(at + 1, rest - stride * i) for i in range(max(first, -down), min(last, up) + 1))
+
+    return reach(0, distance // e)
 
 
 def dense(shape):
