@@ -248,3 +248,55 @@ def test_outputs_in_place_and_refused_ones_on_the_gpu():
         att(x[:4], lens, out=x[1:])
     assert not att(x[:4], lens, out=x[:4])[:].any()  # q itself: no rows, zeros
     s.check()
+
+
+# -------------------------------------------------------------- packed queries
+
+def test_packed_query_rows_are_taken():
+    """One expanded batch may be written where samples have tokens of their
+    own (as far as the device), and nowhere else."""
+    s, lens = KV8Store(4, 64, 4, 1, page_rows=64, device="cpu"), torch.zeros(4, dtype=torch.int32)
+    x = torch.zeros(1, 8, 9, 64).bfloat16().expand(2, -1, -1, -1)
+    q, k, v = x.split([4, 2, 2], 1)
+    out = torch.zeros(1, 4, 9, 64).bfloat16().expand(2, -1, -1, -1)
+    args = dict(rotary=Rotary(_freq(32)), positions=torch.zeros(1, 2, 9, dtype=torch.int64), q=q)
+    for to in (out, q):
+        with pytest.raises(ValueError, match="CUDA device"):
+            s.append(k, v, lens, counts=lens[:2], q_out=to, **args)
+    with pytest.raises(ValueError, match="share memory"):
+        s.append(k, v, lens, q_out=out, **args)
+    with pytest.raises(ValueError, match="share memory"):
+        s.append(k, v, lens, counts=lens[:2], q_out=out[:, :1].expand(2, 4, 9, 64), **args)
+
+
+@gpu
+def test_packed_query_rows():
+    """Ragged prompts packed in one tensor, their queries into another: the
+    rows of a padded output, and the rows of no sample left as they were."""
+    counts, starts, total, D = [40, 1, 0, 97], [2, 42, 42, 44], 143, 128
+    g = torch.Generator().manual_seed(6)
+    x = torch.randn(total, 8, D, generator=g).to(BF16).cuda().transpose(0, 1)[None].expand(4, -1, -1, -1)
+    q, k, v = x.split([4, 2, 2], 1)
+    i32 = lambda t: torch.tensor(t, dtype=torch.int32, device="cuda")  # noqa: E731
+    r, pos = Rotary(_freq(64).cuda()), torch.arange(total, device="cuda").expand(1, 4, total)
+    args = dict(starts=i32(starts), counts=i32(counts), max_count=97, rotary=r, positions=pos, q=q)
+    stores = [KV8Store(8, D, 32, 4, page_rows=32) for _ in range(3)]
+    for s in stores:
+        s.reserve(97)
+    lens = i32([0] * 8)
+    padded = stores[0].append(k, v, lens, **args)
+    packed = torch.full((total, 4, D), 3.0, dtype=BF16, device="cuda")
+    to = packed.transpose(0, 1)[None].expand(4, -1, -1, -1)
+    assert stores[1].append(k, v, lens, q_out=to, **args) is to
+    untouched = torch.ones(total, dtype=torch.bool)
+    for b, (at, n) in enumerate(zip(starts, counts)):
+        assert torch.equal(packed[at:at + n].transpose(0, 1), padded[b, :, at:at + n])
+        untouched[at:at + n] = False
+    assert bool((packed[untouched.cuda()] == 3).all()) and int(untouched.sum()) == 5
+    own = x[0].clone()[None].expand(4, -1, -1, -1)  # in place, within the packed projection
+    q, k, v = own.split([4, 2, 2], 1)
+    stores[2].append(k, v, lens, q_out=q, **{**args, "q": q})
+    assert torch.equal(q[0].transpose(0, 1)[~untouched.cuda()], packed[~untouched.cuda()])
+    for s in stores:
+        s.check()
+        assert torch.equal(s.pool, stores[0].pool) and torch.equal(s.tail_k, stores[0].tail_k)

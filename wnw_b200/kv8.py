@@ -161,7 +161,9 @@ class KV8Store:
         ``positions`` [axes, B, n] rotates the keys before they are held, and
         ``q`` [B, q heads, n, D] into the returned tensor (``q_out``, which
         may be q and shares no memory with k and v, or a new one, contiguous; where a sample has no token a new one is zero and a
-        given one is left as it is).  Returns None without q.  ``stream``:
+        given one is left as it is; of packed tokens a new one is as large as B
+        times all tokens, a given one may be packed too: one expanded batch,
+        the samples' tokens apart from one another).  Returns None without q.  ``stream``:
         launch there, behind what the caller made it wait for.  Problems on the
         device (a segment beyond its pages, an index out of range) set bits
         that ``check()`` reads back.  Not differentiable, like the attention."""
@@ -246,7 +248,8 @@ class KV8Store:
                 raise ValueError(f"q_out {tuple(q_out.shape)} {q_out.dtype}: expected {tuple(qs)} {dtype}")
             else:
                 to = rows(q_out, "q_out", qs)
-                distinct(q_out, "q_out")
+                packed = ragged and B > 1 and q_out.stride(0) == 0
+                distinct(q_out[:1] if packed else q_out, "q_out")
             queries = (qs[1] // H, *rows(q, "q", qs), *to)
         elif q_out is not None:
             raise ValueError("q_out without q")
