@@ -9,6 +9,7 @@ from torch.autograd import forward_ad
 
 from oracle import kv8 as O
 from wnw_b200.kv8 import KV8Attention, KV8Store
+from wnw_b200.kv8_cache import KV8Cache
 from wnw_b200.rotary import Apart, Rotary
 
 gpu = pytest.mark.gpu
@@ -300,3 +301,18 @@ def test_packed_query_rows():
     for s in stores:
         s.check()
         assert torch.equal(s.pool, stores[0].pool) and torch.equal(s.tail_k, stores[0].tail_k)
+
+
+# ------------------------------------------------------------------- KV8Cache
+
+@pytest.mark.parametrize("over,text", [
+    (dict(num_q_heads=36), "group"), (dict(num_q_heads=5), "query heads"), (dict(num_q_heads=0), "group"),
+    (dict(num_kv_heads=0), "query heads"), (dict(head_dim=96), "head_dim"), (dict(code="fp4"), "code"),
+    (dict(page_rows=48), "page_rows"),
+])
+def test_cache_refuses_what_its_attention_does_not_take(over, text):
+    """When it is made, not in the first decode step behind a prefill."""
+    args = dict(num_layers=2, num_kv_heads=4, num_q_heads=32, head_dim=64, device="cpu")
+    KV8Cache(**args)
+    with pytest.raises(ValueError, match=text):
+        KV8Cache(**{**args, **over})

@@ -30,6 +30,23 @@ _CONTIGUOUS = torch.contiguous_format
 _CODES = {"e4m3": N.KV8_E4M3, "int8": N.KV8_INT8}
 
 
+def check_layout(head_dim, page_rows, code):
+    """Refuse what no store holds; returns the blocks of a page."""
+    blocks = page_rows // BLOCK
+    if page_rows % BLOCK or blocks < 1 or blocks & (blocks - 1) or blocks > 64:
+        raise ValueError(f"page_rows {page_rows}: {BLOCK} times a power of two, up to {64 * BLOCK}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim {head_dim}: 64 or 128")
+    if code not in _CODES:
+        raise ValueError(f"code {code!r}: one of {sorted(_CODES)}")
+    return blocks
+
+
+def check_group(group):
+    if not 1 <= int(group) <= 8:
+        raise ValueError(f"group {group}: 1 to 8 query heads a kv head")
+
+
 class KV8Store:
     """One layer's cache: pool, page table and unfinished blocks.
 
@@ -43,11 +60,7 @@ class KV8Store:
 
     def __init__(self, num_segs, head_dim, num_pages, max_pages, page_rows=128, code="e4m3", dtype=torch.bfloat16,
                  device="cuda"):
-        blocks = page_rows // BLOCK
-        if page_rows % BLOCK or blocks < 1 or blocks & (blocks - 1) or blocks > 64:
-            raise ValueError(f"page_rows {page_rows}: {BLOCK} times a power of two, up to {64 * BLOCK}")
-        if head_dim not in (64, 128):
-            raise ValueError(f"head_dim {head_dim}: 64 or 128")
+        blocks = check_layout(head_dim, page_rows, code)
         device = torch.device(device)
         self._init(torch.zeros(num_pages, blocks, 2 * BLOCK * head_dim + N.KV8_PAD, dtype=torch.uint8, device=device),
                    torch.full((num_segs, max_pages), -1, dtype=torch.int32, device=device),
@@ -309,8 +322,7 @@ class KV8Attention:
     ordered anyway (the layers of a model)."""
 
     def __init__(self, store, group, scale, scratch_of=None):
-        if not 1 <= int(group) <= 8:
-            raise ValueError(f"group {group}: 1 to 8 query heads a kv head")
+        check_group(group)
         self.store, self.group, self.scale = store, int(group), float(scale)
         if store.device.type != "cuda":
             raise ValueError(f"the store is on {store.device}: a CUDA device is needed")

@@ -18,11 +18,12 @@ from __future__ import annotations
 import torch
 
 from wnw_b200.flat_cache import FlatVarlenCache
-from wnw_b200.kv8 import KV8Attention, KV8Store
+from wnw_b200.kv8 import KV8Attention, KV8Store, check_group, check_layout
 
 
 class KV8Cache(FlatVarlenCache):
-    """Constructor arguments as ``FlatVarlenCache``; optional: ``code``
+    """Constructor arguments as ``FlatVarlenCache`` (head_dim 64 or 128, one to
+    eight query heads a kv head, a model in bf16 or fp16); optional: ``code``
     ("e4m3" or "int8"), ``page_rows`` (tokens a page), ``max_decode_tokens``
     (pages reserved for decoding at prefill; more are added on demand)."""
 
@@ -33,6 +34,10 @@ class KV8Cache(FlatVarlenCache):
 
     def __init__(self, num_layers, num_kv_heads, num_q_heads, head_dim, device, adapter=None, *, code="e4m3",
                  page_rows=128, max_decode_tokens=1024):
+        check_layout(head_dim, page_rows, code)
+        if num_kv_heads < 1 or num_q_heads % num_kv_heads:
+            raise ValueError(f"{num_q_heads} query heads over {num_kv_heads} kv heads: a multiple of them")
+        check_group(num_q_heads // num_kv_heads)
         super().__init__(num_layers, num_kv_heads, num_q_heads, head_dim, device, adapter)
         if self.device.type == "cuda" and self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
