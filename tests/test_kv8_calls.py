@@ -316,3 +316,50 @@ def test_cache_refuses_what_its_attention_does_not_take(over, text):
     KV8Cache(**args)
     with pytest.raises(ValueError, match=text):
         KV8Cache(**{**args, **over})
+
+
+@gpu
+def test_growth_copies_seldom():
+    """Steps inside the last page leave the pool where it is, and a long
+    generation grows some times, not once in max_decode_tokens."""
+    H, D, prompt, steps = 2, 64, 45, 700
+    cache = KV8Cache(1, H, 4, D, "cuda", page_rows=128, max_decode_tokens=16)
+    cache.setup_audio(torch.tensor([1]), torch.tensor([20]))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, 1, H, prompt + steps, D, generator=g, device="cuda").to(BF16)
+    cache.prefill_after_attn(0, None, None, *x[:, :, :, :prompt])
+    cache.prefill_all_layers_done()
+    q, pools, moved = torch.randn(H, 2, D, generator=g, device="cuda").to(BF16), [cache.stores[0].pool], []
+    for i in range(prompt, prompt + steps):
+        k, v = x[:, :, :, i:i + 1]
+        cache.decode_before_attn(0, k, v)
+        cache.fused_decode_attention(0, q, scale=0.125)
+        cache.decode_all_layers_done()
+        if cache.stores[0].pool is not pools[-1]:
+            pools.append(cache.stores[0].pool)
+            moved.append(i)
+    cache.check()
+    # pages of 128 rows: the first growth where the first page ends, the next where what it added does
+    assert moved[0] == 128 and len(moved) <= 6
+    whole = KV8Store(H, D, H * 6, 6, 128)
+    whole.reserve(prompt + steps)
+    whole.append(*x, torch.zeros(H, dtype=torch.int32, device="cuda"))
+    for s in range(H):
+        for a, b in zip(cache.layer_rows(0, s), whole.dequantize(s, prompt + steps)):
+            assert torch.equal(a, b)
+
+
+@gpu
+def test_growth_within_the_pool_copies_nothing():
+    s = KV8Store(2, 64, 8, 4, page_rows=32)
+    s.reserve(40)
+    x, lens = torch.randn(1, 2, 40, 64, device="cuda").to(BF16), torch.zeros(2, dtype=torch.int32, device="cuda")
+    s.append(x, x, lens)
+    t = s.grown(100)
+    assert t.pool.data_ptr() == s.pool.data_ptr() and t._free == [] and int((t.page_table >= 0).sum()) == 8
+    t.append(x, x, lens + 40)
+    for i in range(2):
+        assert torch.equal(t.dequantize(i, 40)[0][:32], s.dequantize(i, 40)[0][:32])
+    u = t.grown(200)
+    assert u.pool.shape[0] == 14 and torch.equal(u.pool[:8], t.pool)
+    u.check()

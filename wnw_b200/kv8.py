@@ -144,12 +144,13 @@ class KV8Store:
 
     def grown(self, rows):
         """A store with this one's content, and pages for ``rows`` tokens of
-        every segment (the unfinished blocks are shared: use the new one)."""
+        every segment (the unfinished blocks are shared, and the pool where it
+        has pages enough: use the new one)."""
         if self._free is None:
             raise RuntimeError("the pages of a wrapped store are the caller's")
         S, width, have = self.num_segs, -(-int(rows) // self.page_rows), self.pool.shape[0]
         more = max(0, sum(max(0, width - len(o)) for o in self._owned) - len(self._free))
-        pool = torch.cat([self.pool, self.pool.new_zeros(more, *self.pool.shape[1:])])
+        pool = torch.cat([self.pool, self.pool.new_zeros(more, *self.pool.shape[1:])]) if more else self.pool
         table = self.page_table.new_full((S, max(width, self.page_table.shape[1])), -1)
         table[:, :self.page_table.shape[1]] = self.page_table
         s = KV8Store.wrap(pool, table, self.tail_k, self.tail_v, self.code)

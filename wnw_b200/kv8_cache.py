@@ -25,7 +25,8 @@ class KV8Cache(FlatVarlenCache):
     """Constructor arguments as ``FlatVarlenCache`` (head_dim 64 or 128, one to
     eight query heads a kv head, a model in bf16 or fp16); optional: ``code``
     ("e4m3" or "int8"), ``page_rows`` (tokens a page), ``max_decode_tokens``
-    (pages reserved for decoding at prefill; more are added on demand)."""
+    (pages reserved for decoding at prefill; more are added on demand, an eighth
+    of the context at least)."""
 
     #: what the session asks a cache: does it rank audio tokens at prefill,
     #: and does it rotate a decode step's queries and keys itself
@@ -76,8 +77,8 @@ class KV8Cache(FlatVarlenCache):
             self._len = torch.zeros(B * H, dtype=torch.int32, device=self.device)
             self._next = self._counts.repeat_interleave(H)
             self._prompt, self._prompt_rows = S, [S - p for p in self._pads]
-            self._room = S + self.max_decode_tokens
-        pages = -(-self._room // self.page_rows)
+            self._room = self._whole_pages(S + self.max_decode_tokens)
+        pages = self._room // self.page_rows
         store = KV8Store(B * H, D, B * H * pages, pages, self.page_rows, self.code, key_states.dtype, self.device)
         store.reserve(self._room)
         store.append(key_states, value_states, self._len, starts=self._starts, counts=self._counts)
@@ -107,9 +108,13 @@ class KV8Cache(FlatVarlenCache):
         store = self.stores[layer_idx]
         return store.pool, store.pool, self._next, self._prompt + self._step + 1
 
+    def _whole_pages(self, rows):
+        return -(-rows // self.page_rows) * self.page_rows
+
     def _grow(self):
-        """Room for as many decode tokens again, in every layer."""
-        self._room += self.max_decode_tokens
+        """Room for as many decode tokens again, in every layer, and an eighth
+        more at least: each growth copies the layers' content."""
+        self._room = self._whole_pages(self._room + max(self.max_decode_tokens, self._room // 8))
         for l, s in enumerate(self.stores):
             self.stores[l] = s.grown(self._room)
             self._attention[l] = None
