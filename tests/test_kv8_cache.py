@@ -236,3 +236,27 @@ def test_rotary_adapter_refuses_interleaved_sections():
     a = RotaryAdapter(0, 1)
     a.prepare_for_inference(m)
     assert a.rotary.num_axes == 3
+
+
+def test_a_session_that_cannot_be_entered_leaves_the_model_alone():
+    """The second layer's patch fails: the first layer's forward and the rotary
+    module's are the model's own again."""
+    from wnw_b200 import KV8Cache, RotaryAdapter, WnWSession
+    model = _model("cpu")
+
+    class Failing(RotaryAdapter):
+        def attention_meta(self, attn):
+            if attn.layer_idx == 1:
+                raise RuntimeError("no such layer")
+            return super().attention_meta(attn)
+
+    ids = torch.arange(1, 9)[None]
+    with torch.no_grad():
+        want = model(ids).logits
+    session = WnWSession(model, Failing(2, 5), KV8Cache(L, H, HQ, D, "cpu"))
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="no such layer"):
+            session.__enter__()
+        assert session.adapter.rotary is None and not session._orig
+        with torch.no_grad():
+            assert torch.equal(model(ids).logits, want)

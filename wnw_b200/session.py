@@ -40,10 +40,15 @@ class AlgorithmSession:
         self.cache.reset()
         self.adapter.assert_compatible(self.model)
         self._state = self.adapter.prepare_for_inference(self.model)
-        for layer in self.adapter.get_decoder_layers(self.model):
-            attn = layer.self_attn
-            self._orig.append((attn, attn.forward))
-            attn.forward = types.MethodType(self._make_patched_forward(attn), attn)
+        try:
+            for layer in self.adapter.get_decoder_layers(self.model):
+                attn = layer.self_attn
+                forward = types.MethodType(self._make_patched_forward(attn), attn)
+                self._orig.append((attn, attn.forward))
+                attn.forward = forward
+        except BaseException:
+            self.__exit__()  # the model is untouched outside the block, one that could not be entered too
+            raise
         return self
 
     def __exit__(self, *exc):
