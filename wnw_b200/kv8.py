@@ -101,6 +101,7 @@ class KV8Store:
         self.page_rows = pool.shape[1] * BLOCK
         self._index = pool.get_device()
         self._appends = {}  # argument blocks by geometry
+        self._held = pool, tail_k, tail_v  # what an append writes
         self.err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._desc = N.Kv8StoreDesc(N.dtype_code(self.dtype), D, _CODES[code], S, pool.data_ptr(), pool.shape[0],
                                     pool.shape[1], page_table.data_ptr(), page_table.shape[1], tail_k.data_ptr(),
@@ -194,7 +195,8 @@ class KV8Store:
             if len(self._appends) >= 64:
                 self._appends.clear()
             self._appends[key] = base
-        if q_out is not None:
+        given = q_out is not None
+        if given:
             plain(q_out)
             base[2](q_out.data_ptr(), q.data_ptr(), None, k.data_ptr(), None, v.data_ptr())
         index = self._index
@@ -223,7 +225,7 @@ class KV8Store:
             q_in, q_to = q.data_ptr(), q_out.data_ptr()
         launch(index, stream, _APPEND, "wnw_kv8_append_step", base[1], k.data_ptr(), v.data_ptr(), lengths, first, many,
                pos, q_in, q_to)
-        written(self.pool, self.tail_k, self.tail_v, q_out)
+        written(self._held if not given else (*self._held, q_out))
         if stream is not None:
             keep_for(stream, k, v, seg_len, starts, counts, positions, q, q_out, *self._tensors())
             if rotary is not None:
@@ -387,7 +389,7 @@ class KV8Attention:
         launch(s._index, stream, _ATTEND, "wnw_kv8_attn_step", self._args, q.data_ptr(), lengths, out.data_ptr(),
                lse.data_ptr() if return_lse else None, fresh)
         if given is not None:
-            written(given)
+            written((given,))
         if stream is not None:
             keep_for(stream, q, seg_len, out, lse, self.partials, self.counters, *s._tensors())
         return (out, lse) if return_lse else out

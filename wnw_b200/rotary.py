@@ -121,7 +121,7 @@ class Rotary:
         launch(index, stream, _ROTARY, "wnw_rotary_step", base[1], q.data_ptr(), qo.data_ptr(),
                None if k is None else k.data_ptr(), None if ko is None else ko.data_ptr(), positions.data_ptr())
         if out is not None:
-            written(qo, ko)
+            written((qo,) if ko is None else (qo, ko))
         if stream is not None:
             keep_for(stream, q, k, qo, ko, positions, self._freq64, self.axis, self.err)
         return qo, ko
@@ -331,17 +331,17 @@ def made_on(stream, index, make, *args, **kw):
     return t
 
 
-def plain(*outputs):
+def plain(a, b=None):
     """Refuse to write into tensors that carry derivatives: the call would not
     be part of them."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in outputs) or _dual(*outputs):
+    wanted = a is not None and a.requires_grad or b is not None and b.requires_grad
+    if wanted and torch.is_grad_enabled() or forward_ad._current_level >= 0 and _dual(a, b):
         raise ValueError("a given output carries derivatives: write into a detached one, or under no_grad")
 
 
-def written(*tensors):
-    """Tell autograd that a launch has written into the caller's tensors: what
-    was saved of them for a backward pass is refused there."""
-    increment_version([t for t in tensors if t is not None])
+#: tells autograd that a launch has written into the caller's tensors: what was
+#: saved of them for a backward pass is refused there
+written = increment_version
 
 
 def keep_for(stream, *tensors):
