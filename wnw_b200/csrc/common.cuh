@@ -7,6 +7,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/wnw_b200.h"
 
 namespace wnw {
@@ -189,6 +191,19 @@ __device__ inline bool mbar_wait(uint64_t* bar, uint32_t parity, int32_t* err) {
   }
   if (err) atomicOr(err, WNW_DEVERR_MBAR_TIMEOUT);
   return false;
+}
+
+// SMs of the current device
+inline int sm_count() {
+  static std::atomic<int> cached[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int n = cached[dev].load(std::memory_order_relaxed);
+  if (n == 0) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
+    cached[dev].store(n, std::memory_order_relaxed);
+  }
+  return n;
 }
 
 }  // namespace wnw

@@ -4,8 +4,6 @@
 
 #include <cuda_fp8.h>
 
-#include <atomic>
-
 #include "common.cuh"
 
 namespace wnw {
@@ -23,19 +21,6 @@ struct Kv8Rec {
 template <int CODE>
 __host__ __device__ constexpr float kv8_top() {
   return CODE == WNW_KV8_E4M3 ? 448.f : 127.f;
-}
-
-// SMs of the current device
-inline int sm_count() {
-  static std::atomic<int> cached[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int n = cached[dev].load(std::memory_order_relaxed);
-  if (n == 0) {
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) n = 148;
-    cached[dev].store(n, std::memory_order_relaxed);
-  }
-  return n;
 }
 
 // Once a device: lets a kernel take `bytes` of dynamic shared memory

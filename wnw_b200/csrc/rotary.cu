@@ -142,9 +142,10 @@ static wnw_status launch_rotary(const wnw_rotary_args* a, cudaStream_t s) {
   RotarySide k{a->k, a->k_out, a->k_stride_b, a->k_stride_h, a->k_stride_n, a->ko_stride_b, a->ko_stride_h,
                a->ko_stride_n, a->num_kv_heads};
   const int64_t total = int64_t(a->batch) * a->tokens;
-  // tokens of a CTA: as many as leave three CTAs an SM, and a thread for each place
+  // tokens of a CTA: doubled while the grid has more than three CTAs an SM
+  // (then it has 1.5 at least) and each place a thread
   int per = 1;
-  while (per < kRotTokens && total > int64_t(per) * 444 && 2 * per * (a->head_dim / 16) <= kRotThreads) per *= 2;
+  while (per < kRotTokens && total > int64_t(per) * 3 * sm_count() && 2 * per * (a->head_dim / 16) <= kRotThreads) per *= 2;
   const size_t smem = sizeof(float2) * per * (a->rope.rot / 2);
   const int64_t grid = (total + per - 1) / per;
   WNW_CHECK_ARG(grid < (int64_t(1) << 31), "too many tokens");
