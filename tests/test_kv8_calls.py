@@ -1,6 +1,7 @@
 """Calls of the 8-bit cache and the rotation at the borders of what their
 documentation allows: numbers near 31 bits, outputs that share memory,
 derivatives, growth."""
+import ctypes
 import random
 
 import pytest
@@ -8,6 +9,7 @@ import torch
 from torch.autograd import forward_ad
 
 from oracle import kv8 as O
+from wnw_b200 import native as N
 from wnw_b200.kv8 import KV8Attention, KV8Store
 from wnw_b200.kv8_cache import KV8Cache
 from wnw_b200.rotary import Apart, Rotary
@@ -363,3 +365,16 @@ def test_growth_within_the_pool_copies_nothing():
     u = t.grown(200)
     assert u.pool.shape[0] == 14 and torch.equal(u.pool[:8], t.pool)
     u.check()
+
+
+def test_numbers_of_pages_that_wrap_around_are_refused():
+    """Checked on the host: 2^58 pages of 64 blocks are 2^64."""
+    for pages in (1 << 58, (1 << 57) + 1, 1 << 31):
+        d = N.Kv8StoreDesc(dtype=N.BF16, head_dim=64, code=0, num_segs=2, pool=4096, num_pages=pages, page_blocks=64,
+                           page_table=4096, max_pages=2, tail_k=4096, tail_v=4096, err=4096)
+        a = N.Kv8AppendArgs(store=d, batch=1, num_kv_heads=2, tokens=4, max_count=4, seg_len=4096, k=4096, v=4096)
+        b = N.Kv8AttnArgs(store=d, group=4, q=4096, seg_len=4096, out=4096, scale=1.0, partials=4096,
+                          partial_floats=1 << 30, counters=4096)
+        for call, args in ((N.lib.wnw_kv8_append, a), (N.lib.wnw_kv8_attn, b)):
+            assert call(ctypes.byref(args), None) == N.WNW_ERR_INVALID
+            assert "blocks" in N.lib.wnw_last_error().decode()

@@ -44,7 +44,8 @@ inline wnw_status check_kv8_store(const wnw_kv8_store& s) {
   WNW_CHECK_ARG(s.num_segs > 0 && s.num_pages >= 0 && s.max_pages >= 0, "bad segment or page counts");
   WNW_CHECK_ARG(s.page_blocks >= 1 && s.page_blocks <= 64 && (s.page_blocks & (s.page_blocks - 1)) == 0,
                 "page_blocks %d: a power of two up to 64", s.page_blocks);
-  WNW_CHECK_ARG(s.num_pages * s.page_blocks < (int64_t(1) << 31), "2^31 blocks or more");
+  WNW_CHECK_ARG(s.num_pages < (int64_t(1) << 31) && s.num_pages * s.page_blocks < (int64_t(1) << 31),
+                "2^31 blocks or more");
   WNW_CHECK_ARG(int64_t(s.max_pages) * s.page_blocks * kKv8Block < (int64_t(1) << 31), "2^31 tokens a segment or more");
   WNW_CHECK_ARG((s.pool || s.num_pages == 0) && (s.page_table || s.max_pages == 0) && s.tail_k && s.tail_v && s.err,
                 "null pointer argument");
