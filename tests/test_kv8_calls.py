@@ -378,3 +378,12 @@ def test_numbers_of_pages_that_wrap_around_are_refused():
         for call, args in ((N.lib.wnw_kv8_append, a), (N.lib.wnw_kv8_attn, b)):
             assert call(ctypes.byref(args), None) == N.WNW_ERR_INVALID
             assert "blocks" in N.lib.wnw_last_error().decode()
+
+
+@pytest.mark.parametrize("hq,hk", [(1 << 30, 1 << 30), ((1 << 31) - 1, 1), ((1 << 31) - 1, (1 << 31) - 1), (1 << 20, 1)])
+def test_numbers_of_heads_that_wrap_around_are_refused(hq, hk):
+    a = N.RotaryArgs(dtype=N.BF16, head_dim=64, batch=1, tokens=2, num_q_heads=hq, num_kv_heads=hk, q=4096, q_out=4096,
+                     k=8192, k_out=8192, err=4096,
+                     rope=N.Rope(rot=64, num_axes=1, inv_freq=4096, axis=4096, pos=4096))
+    assert N.lib.wnw_rotary(ctypes.byref(a), None) == N.WNW_ERR_INVALID
+    assert "heads" in N.lib.wnw_last_error().decode()

@@ -168,7 +168,8 @@ extern "C" wnw_status wnw_rotary(const wnw_rotary_args* a, void* stream) {
                 "head_dim %d: a multiple of 16 up to 512", a->head_dim);
   WNW_CHECK_ARG(a->batch >= 0 && a->tokens >= 0 && a->num_q_heads >= 0 && a->num_kv_heads >= 0, "negative size");
   WNW_CHECK_ARG(a->err != nullptr, "null error word");
-  if (a->batch == 0 || a->tokens == 0 || a->num_q_heads + a->num_kv_heads == 0) return WNW_OK;
+  const int64_t heads = int64_t(a->num_q_heads) + a->num_kv_heads;
+  if (a->batch == 0 || a->tokens == 0 || heads == 0) return WNW_OK;
   WNW_CHECK_ARG((a->num_q_heads == 0 || (a->q && a->q_out)) && (a->num_kv_heads == 0 || (a->k && a->k_out)),
                 "null pointer argument");
   const int e16 = a->dtype == WNW_F32 ? 4 : 8;
@@ -180,7 +181,7 @@ extern "C" wnw_status wnw_rotary(const wnw_rotary_args* a, void* stream) {
                                          strides_ok(a->k_stride_b, a->k_stride_h, a->k_stride_n, e16) &&
                                          strides_ok(a->ko_stride_b, a->ko_stride_h, a->ko_stride_n, e16)),
                 "k and its output need 16-byte aligned rows");
-  WNW_CHECK_ARG(int64_t(a->num_q_heads + a->num_kv_heads) * a->head_dim <= (1 << 26), "too many heads");
+  WNW_CHECK_ARG(heads * a->head_dim <= (1 << 26), "too many heads");
   const wnw_status st = check_rope(a->rope, a->head_dim);
   if (st != WNW_OK) return st;
   WNW_CHECK_ARG(a->rope.rot > 0, "rotation of no dimensions");
