@@ -99,3 +99,27 @@ def test_small_dimensions_beside_a_large_one(code, dtype, D, n):
     out, lse = KV8Attention(store, 4, 2.0 ** 8)(q.cuda(), lens, return_lse=True)
     _check(store, q, n, 2.0 ** 8, out, lse, range(3))
     store.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("size", [2.0 ** 20, 2.0 ** 26, 2.0 ** 30])
+def test_equal_scores_of_any_size(dtype, size):
+    """Equal keys weigh the same, in blocks and in the unfinished one, however
+    large their scores: the output is the values' mean."""
+    n, D = 73, 64
+    k = torch.zeros(2, n, D, dtype=dtype)
+    k[..., :2] = 1.0
+    v = torch.zeros(2, n, D, dtype=dtype)
+    v[:, :64, 0], v[:, 64:, 1] = 1.0, 1.0
+    store, lens = _filled(k, v, "int8")
+    store.scales()[..., 0] = 2.0 ** -7  # 127 codes of a key of 127 / 128: scores exact in fp32
+    store.tail_k[:, 0, :, :2] = 127 / 128
+    q = torch.zeros(2, 1, D, dtype=dtype)
+    q[..., 0] = 1.0
+    out, _ = KV8Attention(store, 1, size)(q.cuda(), lens, return_lse=True)
+    want = torch.zeros(2, 1, D, dtype=torch.float64)
+    want[..., 0], want[..., 1] = 64 / n, 9 / n
+    eps = torch.finfo(dtype).eps
+    # the output's rounding, and the values' scale (2^-20); both keys' scores are the same number
+    assert bool(((out.cpu().double() - want).abs() <= (eps / 2 + 2.0 ** -12) * want).all()), out[..., :2]
+    store.check()

@@ -54,7 +54,7 @@ constexpr int kK8Threads = 256;
 constexpr int kK8Warps = 8;
 constexpr float kK8Log2e = 1.4426950408889634f;
 constexpr float kK8Ln2 = 0.6931471805599453f;
-constexpr float kK8Up = 14.f, kK8Down = 1.f / 16384.f;  // fp16 probabilities are held 2^14 up
+constexpr float kK8Up = 16384.f, kK8Down = 1.f / 16384.f;  // fp16 probabilities are held 2^14 up
 
 template <int D>
 constexpr int k8_stages() {
@@ -403,8 +403,9 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
       // 16-token steps in which a lane's 8 value bytes lie in order
       const int tok = 8 * (gid >> 1) + (gid & 1);
 
-      // scores -> probabilities times 2^up (fp32, in sc), the running state, al0 / al1
-      auto softmax = [&](float (&sc)[2][4], float& al0, float& al1, float up, float down) {
+      // scores -> probabilities times `up` (fp32, in sc), the running state, al0 / al1.  (2^14 is not
+      // taken into the exponent: beyond 2^24 a score less 14 is not that)
+      auto softmax = [&](float (&sc)[2][4], float& al0, float& al1, float up) {
         float mx0 = fmaxf(fmaxf(sc[0][0], sc[0][2]), fmaxf(sc[1][0], sc[1][2]));
         float mx1 = fmaxf(fmaxf(sc[0][1], sc[0][3]), fmaxf(sc[1][1], sc[1][3]));
 #pragma unroll
@@ -417,18 +418,21 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
         const float b0 = mx0 == -INFINITY ? 0.f : mx0, b1 = mx1 == -INFINITY ? 0.f : mx1;
         al0 = ex2(m0 - b0);
         al1 = ex2(m1 - b1);
-        const float u0 = b0 - up, u1 = b1 - up;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          sc[i][0] = ex2(sc[i][0] - u0);
-          sc[i][1] = ex2(sc[i][1] - u1);
-          sc[i][2] = ex2(sc[i][2] - u0);
-          sc[i][3] = ex2(sc[i][3] - u1);
+          sc[i][0] = ex2(sc[i][0] - b0);
+          sc[i][1] = ex2(sc[i][1] - b1);
+          sc[i][2] = ex2(sc[i][2] - b0);
+          sc[i][3] = ex2(sc[i][3] - b1);
         }
         m0 = mx0;
         m1 = mx1;
-        l0 = fmaf(l0, al0, ((sc[0][0] + sc[0][2]) + (sc[1][0] + sc[1][2])) * down);
-        l1 = fmaf(l1, al1, ((sc[0][1] + sc[0][3]) + (sc[1][1] + sc[1][3])) * down);
+        l0 = l0 * al0 + ((sc[0][0] + sc[0][2]) + (sc[1][0] + sc[1][2]));
+        l1 = l1 * al1 + ((sc[0][1] + sc[0][3]) + (sc[1][1] + sc[1][3]));
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[i][e] *= up;
       };
 
       __syncwarp();
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
         // range needs no 2^14; 11 + 11 for fp16)
         constexpr bool kHalf = std::is_same<T, __half>::value;
         float al0, al1;
-        softmax(sc, al0, al1, kHalf ? kK8Up : 0.f, kHalf ? kK8Down : 1.f);
+        softmax(sc, al0, al1, kHalf ? kK8Up : 1.f);
         uint32_t pb[4], pr[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -537,7 +541,7 @@ __global__ void __launch_bounds__(kK8Threads, 1) kv8_attn_kernel(const __grid_co
             sc[i][3] = c[3] * k1;
           }
           float al0, al1;
-          softmax(sc, al0, al1, kK8Up, kK8Down);
+          softmax(sc, al0, al1, kK8Up);
           // (a block of values below 2^-103 loses bits of its scale here)
           const float vs = scl.y * kK8Down;
           uint32_t pb[4], pr[4];  // probabilities, and what their rounding left
