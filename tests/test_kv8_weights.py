@@ -123,3 +123,31 @@ def test_equal_scores_of_any_size(dtype, size):
     # the output's rounding, and the values' scale (2^-20); both keys' scores are the same number
     assert bool(((out.cpu().double() - want).abs() <= (eps / 2 + 2.0 ** -12) * want).all()), out[..., :2]
     store.check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n", [20, 31, 84])
+def test_weights_of_values_that_cancel(dtype, n):
+    """Values of 1 and -1 whose sum is small beside their number: what the
+    weights' own rounding leaves is not hidden behind the output's.  A weight
+    is off by 2^-22 of itself however it is held, by its exponential (2^-21)
+    and its score (2^-20 of the terms' magnitudes, twice)."""
+    g = torch.Generator().manual_seed(n)
+    S, G, D = 40, 8, 128
+    k = torch.randn(S, n, D, generator=g).to(dtype)
+    v = (1 - 2 * torch.randint(0, 2, (S, n, D), generator=g)).to(dtype)
+    q = torch.randn(S, G, D, generator=g).to(dtype)
+    store, lens = _filled(k, v, "int8")
+    out = KV8Attention(store, G, D ** -0.5)(q.cuda(), lens)
+    eps, small = torch.finfo(dtype).eps, 0
+    for s in range(S):
+        kk, vv = (x.cpu().double() for x in store.dequantize(s, n))
+        x = q[s].double()
+        want, _, pv = O.attention(x, kk, vv, D ** -0.5)
+        ds = 2.0 ** -20 * float((x.abs() @ kk.abs().t()).max()) * D ** -0.5
+        tol = eps / 2 * want.abs() * (1 + 2.0 ** -7) + (2.0 ** -22 + 2.0 ** -21 + 2 * ds + 2.0 ** -20) * pv + 2.0 ** -25
+        small += int((want.abs() < 2.0 ** -9).sum())
+        off = (out[s].cpu().double() - want).abs()
+        assert bool((off <= tol).all()), (s, float((off / tol).max()))
+    assert small > 100
+    store.check()
