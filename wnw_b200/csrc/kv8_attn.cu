@@ -22,26 +22,29 @@
 // in fp16: exact for fp16 models, for bf16 ones down to 2^-32 of the head's
 // largest dimension (11 bits, bf16's 8 fit; what fp16 cannot hold below that
 // is under 2^-40 of it).  Codes become fp16 exactly, so the first product
-// rounds in its fp32 accumulation only.  The second takes the
-// probabilities as two fp16 terms, 22 bits, so outputs are as near as with
-// fp32 ones (one term, 2^-11 of each: as much as an fp16 output's own
-// rounding, an eighth of a bf16 one's; 1 to 3 % faster: two requests of 120k
-// tokens 85.4 us, one of 15k 14.6).  They are held 2^14 above the running
-// maximum's, so that what fp16 loses stays under 2^-39 of it (unscaled, 255
-// equal tokens 17 nats under a first one of value zero vanished); the values'
-// scale takes the 2^14 back.  Both run as m16n8k16 tensor-core products with the head
-// group as n: a query token has G rows only, the tensor pipe is busy 16-19 %
-// of the time and its shape does not bound.  The value scale is applied to
-// each block's product in fp32, whatever its range.
+// rounds in its fp32 accumulation only.  The second takes the probabilities
+// of full blocks as two fp16 terms, 22 bits, so outputs are as near as with
+// fp32 ones (one term, 2^-11 of each, is as much as an fp16 output's own
+// rounding and an eighth of a bf16 one's; it was 1 to 3 % faster: two requests
+// of 120k tokens 85.4 us, one of 15k 14.6).  They are held 2^14 above the
+// running maximum's, so that what fp16 loses stays under 2^-39 of it
+// (unscaled, 255 equal tokens 17 nats under a first one of value zero
+// vanished); the values' scale takes the 2^14 back.  The unfinished block's
+// are two terms of its type: 16 bits in bf16, 2^-8 of its output's rounding (a
+// third term cost calls of a few tokens 3 to 5 %).  Both products run as
+// m16n8k16 tensor-core ones with the head group as n: a query token has G
+// rows only, the tensor pipe is busy 23 to 29 % of the time and its shape does
+// not bound.  The value scale is applied to each block's product in fp32.
 //
 // Measured (e4m3, bf16, head_dim 128, groups of 4, 6,547 GB/s copy rate): two
-// requests of 120k tokens 85.8 us = 5.7 TB/s of codes (87 %); 32 ragged
-// requests of 6k tokens in int8, groups of 7, 48.9 us = 4.8 TB/s (SMs reach
+// requests of 120k tokens 86.6 us = 5.7 TB/s of codes (87 %); 32 ragged
+// requests of 6k tokens in int8, groups of 7, 48.3 us = 4.9 TB/s (SMs reach
 // the end of their stretches up to 10 us apart); one request of 15k tokens
-// 14.7 us, of which about 4 pass before the first record lands and 6 in the
-// merge and its arrivals; 32 segments of 40 tokens 8 us.  With `fresh` the
-// time ahead of the records hides behind the append (12.5 and 45.2 us).  The
-// 16-bit kernel takes 16.8, 155.6 and 82.8 us for these lengths.
+// 15.1 us, of which about 4 pass before the first record lands and 6 in the
+// merge and its arrivals; 32 segments of 40 tokens 8 us, 3 segments of 9
+// tokens, which nothing merges, 3.3.  With `fresh` the time ahead of the
+// records hides behind the append (81.3, 44.2, 12.9 and 6.8 us).  The 16-bit
+// kernel takes 154.7, 83.5 and 16.9 us for the first three lengths.
 #include <atomic>
 #include <type_traits>
 
