@@ -164,7 +164,8 @@ def test_outputs_of_the_cache_that_carry_derivatives_are_refused():
     kv = torch.zeros(1, 2, 3, 64, dtype=BF16, device="cuda")
     q, pos = torch.zeros(1, 4, 3, 64, dtype=BF16, device="cuda"), torch.zeros(1, 3, dtype=torch.int64, device="cuda")
     with pytest.raises(ValueError, match="carries derivatives"):
-        s.append(kv, kv, lens, rotary=Rotary(_freq(32).cuda()), positions=pos, q=q, q_out=torch.empty_like(q).requires_grad_())
+        s.append(kv, kv, lens, rotary=Rotary(_freq(32).cuda()), positions=pos, q=q,
+                 q_out=torch.empty_like(q).requires_grad_())
     one = torch.zeros(2, 2, 64, dtype=BF16, device="cuda")
     with pytest.raises(ValueError, match="carries derivatives"):
         KV8Attention(s, 2, 0.1)(one, lens, out=torch.empty_like(one).requires_grad_())
@@ -208,7 +209,8 @@ def test_outputs_that_share_memory_with_other_tensors_are_refused():
     qkv = torch.zeros(2, 5, 8, 64).transpose(1, 2)
     q, k, v = qkv.split([4, 2, 2], 1)
     two = torch.zeros(2, 4, 6, 64)
-    for ins, outs in (((k, v), (v, k)), ((k, v), (k, k)), ((k, v), (torch.zeros_like(k), k)), ((k, v), (v, torch.zeros_like(v))),
+    for ins, outs in (((k, v), (v, k)), ((k, v), (k, k)), ((k, v), (torch.zeros_like(k), k)),
+                      ((k, v), (v, torch.zeros_like(v))),
                       ((two[:, :, :5], None), (two[:, :, 1:], None)),
                       ((two[:, :, :4], None), (two.view(-1)[:2 * 4 * 4 * 64].view(2, 4, 4, 64), None))):
         with pytest.raises(ValueError, match="shares memory"):
@@ -246,10 +248,11 @@ def test_outputs_in_place_and_refused_ones_on_the_gpu():
     assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(v, left)
     s = KV8Store(4, 64, 4, 1, page_rows=32)
     s.reserve(32)
-    att, lens, x = KV8Attention(s, 2, 0.1), torch.zeros(4, dtype=torch.int32, device="cuda"), torch.randn(5, 2, 64, device="cuda").to(BF16)
+    att, lens = KV8Attention(s, 2, 0.1), torch.zeros(4, dtype=torch.int32, device="cuda")
+    x = torch.randn(5, 2, 64, device="cuda").to(BF16)
     with pytest.raises(ValueError, match="shares memory"):
         att(x[:4], lens, out=x[1:])
-    assert not att(x[:4], lens, out=x[:4])[:].any()  # q itself: no rows, zeros
+    assert not att(x[:4], lens, out=x[:4]).any()  # q itself: no rows, zeros
     s.check()
 
 
@@ -380,10 +383,76 @@ def test_numbers_of_pages_that_wrap_around_are_refused():
             assert "blocks" in N.lib.wnw_last_error().decode()
 
 
-@pytest.mark.parametrize("hq,hk", [(1 << 30, 1 << 30), ((1 << 31) - 1, 1), ((1 << 31) - 1, (1 << 31) - 1), (1 << 20, 1)])
+@pytest.mark.parametrize("hq,hk", [(1 << 30, 1 << 30), ((1 << 31) - 1, 1), ((1 << 31) - 1, (1 << 31) - 1),
+                                   (1 << 20, 1)])
 def test_numbers_of_heads_that_wrap_around_are_refused(hq, hk):
     a = N.RotaryArgs(dtype=N.BF16, head_dim=64, batch=1, tokens=2, num_q_heads=hq, num_kv_heads=hk, q=4096, q_out=4096,
                      k=8192, k_out=8192, err=4096,
                      rope=N.Rope(rot=64, num_axes=1, inv_freq=4096, axis=4096, pos=4096))
     assert N.lib.wnw_rotary(ctypes.byref(a), None) == N.WNW_ERR_INVALID
     assert "heads" in N.lib.wnw_last_error().decode()
+
+
+# ------------------------------------------------- captured, and large and small heads
+
+@gpu
+def test_captured_steps_with_fresh_tokens():
+    """A decode step as a loop runs it, the attention early behind the append,
+    captured once and replayed over growing sequences that finish blocks and
+    begin pages: the bits of one that waits."""
+    B, H, G, D, n, steps = 3, 2, 4, 64, 57, 80
+    g = torch.Generator(device="cuda").manual_seed(8)
+    store = KV8Store(B * H, D, B * H * 5, 5, page_rows=32)
+    store.reserve(n + steps + 2)
+    r, att, other = Rotary(_freq(32).cuda()), *(KV8Attention(store, G, 0.125) for _ in range(2))
+    lens = torch.tensor([0, 31, 32, 57, 5, 40], dtype=torch.int32, device="cuda")
+    kv = torch.randn(B * H, 1, n, D, generator=g, device="cuda").to(BF16)
+    KV8Store.wrap(store.pool, store.page_table, store.tail_k, store.tail_v).append(kv, kv, lens * 0, counts=lens)
+    x = torch.randn(B, H * (G + 2), 1, D, generator=g, device="cuda").to(BF16)
+    new, pos = lens + 1, torch.full((1, B, 1), 57, dtype=torch.int64, device="cuda")
+
+    def step():
+        q = store.append(x[:, H * G:H * G + H], x[:, -H:], lens, rotary=r, positions=pos, q=x[:, :H * G])
+        out, lse = att(q.view(B * H, G, D), new, return_lse=True, fresh=1)
+        lens.add_(1)
+        new.add_(1)
+        pos.add_(1)
+        return q, out, lse
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, out, lse = step()
+    for _ in range(steps):
+        x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        graph.replay()
+        want = other(q.view(B * H, G, D), lens, return_lse=True)  # lens: the step's new ones by now
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    store.check()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, BF16])
+@pytest.mark.parametrize("D,rot,Hq,Hk,n", [(512, 512, 3, 1, 700), (512, 16, 1, 2, 9), (16, 16, 40, 0, 3000),
+                                          (496, 240, 2, 2, 301), (32, 16, 1, 1, 1), (128, 128, 1, 0, 1)])
+def test_rotary_large_and_small_heads(dtype, D, rot, Hq, Hk, n):
+    """Tolerance as derived in test_rotary.py: the type's rounding, and 2^-22
+    of both magnitudes for the fp32 cosine, sine, products and sum."""
+    g = torch.Generator().manual_seed(D + n)
+    r = Rotary(_freq(rot // 2).cuda())
+    pos = torch.randint(0, 10 ** 6, (1, 2, n), generator=g)
+    x = [torch.randn(2, h, n, D, generator=g).to(dtype) for h in (Hq, Hk)]
+    got = r(x[0].cuda(), x[1].cuda() if Hk else None, pos.cuda())
+    for y, z in zip(got, x[:2 if Hk else 1]):
+        want = O.rotate(z, pos, r.inv_freq.cpu(), [0] * (rot // 2))
+        m = z.double().abs()
+        both = m[..., :rot // 2] + m[..., rot // 2:rot]
+        mag = torch.cat([both, both, torch.zeros_like(m[..., rot:])], -1)
+        tiny = {torch.float32: 2.0 ** -150, torch.float16: 2.0 ** -25, BF16: 2.0 ** -134}[dtype]
+        tol = torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2.0 ** -7) + 2.0 ** -22 * mag + tiny
+        assert bool(((y.cpu().double() - want).abs() <= tol).all())
+    r.check()

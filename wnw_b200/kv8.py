@@ -174,14 +174,16 @@ class KV8Store:
         are starts[b] ... starts[b] + counts[b] of the n, ``max_count`` (host)
         at least the largest count.  ``rotary`` (a ``Rotary``) with
         ``positions`` [axes, B, n] rotates the keys before they are held, and
-        ``q`` [B, q heads, n, D] into the returned tensor (``q_out``, which
-        may be q and shares no memory with k and v, or a new one, contiguous; where a sample has no token a new one is zero and a
-        given one is left as it is; of packed tokens a new one is as large as B
-        times all tokens, a given one may be packed too: one expanded batch,
-        the samples' tokens apart from one another).  Returns None without q.  ``stream``:
-        launch there, behind what the caller made it wait for.  Problems on the
-        device (a segment beyond its pages, an index out of range) set bits
-        that ``check()`` reads back.  Not differentiable, like the attention."""
+        ``q`` [B, q heads, n, D] into the returned tensor: ``q_out``, which may
+        be q and shares no memory with k and v, or a new one, contiguous.
+        Where a sample has no token a new one is zero and a given one is left
+        as it is.  Of packed tokens a new one is as large as B times all
+        tokens; a given one may be packed too, one expanded batch, where the
+        samples' tokens are apart from one another.  Returns None without q.
+        ``stream``: launch there, behind what the caller made it wait for.
+        Problems on the device (a segment beyond its pages, an index out of
+        range) set bits that ``check()`` reads back.  Not differentiable, like
+        the attention."""
         # the checks and the argument block depend on shapes, strides, types and
         # the rotation alone: each geometry is looked at once, a call brings its
         # pointers

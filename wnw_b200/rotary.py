@@ -84,10 +84,11 @@ class Rotary:
         dimensions of any stride; positions [axes, B, n] ([B, n] with one
         axis), int32 or int64: below 2^29 in magnitude their angles are exact,
         above (up to 2^51) they carry a rounding to 64 bits.  ``inverse``
-        applies the transposed rotation: the gradient of the forward one.  ``out``: (q, k) to write, each of
-        which may be its own input and shares no memory with the other tensors.  ``stream``: launch there, behind what the
-        caller made it wait for.  Differentiable with respect to q and k,
-        backward and forward (dual tensors)."""
+        applies the transposed rotation: the gradient of the forward one.
+        ``out``: (q, k) to write, each of which may be its own input and shares
+        no memory with the other tensors.  ``stream``: launch there, behind
+        what the caller made it wait for.  Differentiable with respect to q and
+        k, backward and forward (dual tensors)."""
         if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)) or _dual(q, k):
             if out is not None or stream is not None:
                 raise ValueError("out and stream cannot be given where gradients are wanted")
@@ -110,7 +111,8 @@ class Rotary:
             self._calls[key] = base
         index = self._index
         if out is not None:
-            base[2](qo.data_ptr(), q.data_ptr(), None if ko is None else ko.data_ptr(), None if k is None else k.data_ptr())
+            base[2](qo.data_ptr(), q.data_ptr(), None if ko is None else ko.data_ptr(),
+                    None if k is None else k.data_ptr())
         if out is None:
             qo = made_on(stream, index, torch.empty_like, q, memory_format=torch.contiguous_format)
             if k is not None:
@@ -249,20 +251,17 @@ class Apart:
                     continue
                 own = i == j - 1 and j % 2 == 1 and all(
                     s == t or n == 1 for s, t, n in zip(a.stride(), b.stride(), a.shape))
-                la, lb = ((t.shape, t.stride(), t.element_size()) for t in (a, b))
-                self._pairs.append((i, j, _span(la), _span(lb), own, {}, la, lb, name))
+                la, lb = ((tuple(t.shape), t.stride(), t.element_size()) for t in (a, b))
+                self._pairs.append((i, j, _span(la), _span(lb), own, la, lb, name))
 
     def __call__(self, *at):
-        for i, j, after, before, own, known, la, lb, name in self._pairs:
+        seen = []  # (in place, several pairs are the same two)
+        for i, j, after, before, own, la, lb, name in self._pairs:
             d = at[j] - at[i]
-            if -before < d < after and not (own and d == 0):
-                meet = known.get(d)
-                if meet is None:
-                    if len(known) > 64:
-                        known.clear()
-                    meet = known[d] = _meet(la, lb, d)
-                if meet:
+            if -before < d < after and not (own and d == 0) and (la, lb, d) not in seen:
+                if _meet(la, lb, d):
                     raise ValueError(f"{name}: shares memory with another tensor of the call")
+                seen.append((la, lb, d))
 
 
 def _span(layout):
